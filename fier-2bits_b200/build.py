@@ -51,7 +51,8 @@ def _run(cmd, verbose):
 
 
 def build_c_library(force: bool = False, verbose: bool = False) -> Path:
-    headers = [CSRC / "common.cuh", CSRC / "score_core.cuh", CSRC / "paged_core.cuh", INCLUDE / "popkv_b200.h"]
+    headers = [CSRC / "common.cuh", CSRC / "score_core.cuh", CSRC / "paged_core.cuh",
+               CSRC / "key_range.h", INCLUDE / "popkv_b200.h"]
     deps = [CSRC / s for s in CUDA_SOURCES] + headers
     if not force and not _stale(C_LIB, deps):
         return C_LIB

@@ -7,7 +7,7 @@
 //  * select: one CTA per query head holds the row's order keys in registers and finds the key
 //    of rank budget - 1 by histograms of 2048 bins over the range that is left: first the row's own
 //    [least, largest], which spreads the keys over the bins whatever their exponents are, then the
-//    bin that holds the rank, until that bin is taken whole (two rounds as a rule).  The picks are
+//    bin that holds the rank, until that bin is taken whole (two rounds as a rule, three at most).  The picks are
 //    written as a bitmap; the last query head of a KV head merges its group's bitmaps into an
 //    ascending page list with head masks.  Latency-bound: 8.5 us for 32 rows of 2048 pages, of
 //    which the launch is 3, the keys' arrival 1.5, the search 2 and ticket and merge 2; 256 rows of
@@ -15,6 +15,7 @@
 #include <cmath>
 #include <type_traits>
 
+#include "key_range.h"
 #include "paged_core.cuh"
 
 namespace popkv {
@@ -178,7 +179,7 @@ __global__ void __launch_bounds__(NT) paged_select_kernel(SelectArgs a) {
     pdl_wait();
     constexpr int kWarps = NT / 32;
     constexpr int kRounds = KPT > 0 ? KPT : 1;
-    constexpr int kBins = 2048, kPer = kBins / NT;  // bins per thread in the scan
+    constexpr int kBins = 1 << KeyRange::kBits, kPer = kBins / NT;  // bins per thread in the scan
     __shared__ __align__(16) uint32_t s_hist[kBins];
     __shared__ uint32_t s_warp[2][kWarps];
     __shared__ uint32_t s_ties[kRounds * kWarps];
@@ -229,12 +230,12 @@ __global__ void __launch_bounds__(NT) paged_select_kernel(SelectArgs a) {
             thr = 0xffffffffu;
             take = 0u;
         } else if (want < count) {
-            uint32_t left = want;  // rank wanted among the keys of [lo, hi]
-            for (;;) {
-                const int bits = 32 - __clz(hi - lo);
-                const int shift = bits > 11 ? bits - 11 : 0;
+            uint32_t left = want;  // rank wanted among the keys of the range
+            KeyRange range{lo, hi};
+            for (int step = 1;; ++step) {
+                const int shift = range.shift();
                 each([&](uint32_t k) {
-                    if (k >= lo && k <= hi) atomicAdd(s_hist + ((k - lo) >> shift), 1u);
+                    if (range.holds(k)) atomicAdd(s_hist + range.bin(k, shift), 1u);
                 });
                 __syncthreads();
                 // Suffix sums: thread t owns bins kPer t ..; keys in the bins above its own.
@@ -264,15 +265,14 @@ __global__ void __launch_bounds__(NT) paged_select_kernel(SelectArgs a) {
                     s_hist[kPer * tid + i] = 0u;  // for the next round
                 }
                 __syncthreads();
-                lo += s_pick[0] << shift;
+                range.keep(s_pick[0], shift);
                 left -= s_pick[1];
                 const bool whole = left == s_pick[2];  // the bin is taken whole
-                if (whole || shift == 0) {
-                    thr = lo;
+                if (whole || shift == 0 || step == KeyRange::kSteps) {  // the last step's bins hold one key each
+                    thr = range.lo;
                     take = whole ? 0xffffffffu : left;
                     break;
                 }
-                hi = min(hi, lo + ((1u << shift) - 1u));
                 // The next writes of s_warp and s_pick come after two more barriers.
             }
         }

@@ -402,7 +402,8 @@ def paged_score(q: torch.Tensor, cache, block_table: torch.Tensor, lengths: torc
     """Upper bound of q.k over every page: sum_d max(q_d lo_d, q_d hi_d), fp32 [B, QH, columns].
 
     The Quest score (popkv.py:167-178) over the bounds that the writers keep; columns
-    past the sequence's last page and unmapped ones get -inf.
+    past the sequence's last page and unmapped ones get -inf.  A page whose bounds hold a NaN or an
+    infinity scores NaN or +inf, above every number.
     """
     if q.ndim != 3 or not q.is_cuda or not q.is_contiguous():
         raise ValueError("queries must be contiguous CUDA [batch, query heads, head dim]")

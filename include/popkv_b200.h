@@ -471,6 +471,8 @@ int popkv_paged_attention(const void* q, const popkv_paged_cache* cache, const i
  * scores[b, h, i] = sum_d max(q_d lo_d, q_d hi_d) over the bounds of the page in table
  * column i, an upper bound of q . k over the page's tokens; fp32 [batch, q_heads,
  * table_width].  Columns past the sequence's last page and unmapped ones get -infinity.
+ * A page with a NaN bound scores NaN, one with an infinite bound NaN or +infinity (0 times infinity
+ * where the query's sign picks the other bound): both above every number in a selection.
  */
 int popkv_paged_score(const void* q, const popkv_paged_cache* cache, const int32_t* table,
                       int64_t table_stride, int64_t table_width, const int32_t* lengths,
