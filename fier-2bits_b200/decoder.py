@@ -403,7 +403,7 @@ class GraphedDecoder:
             k, v = _layer_cache(cache, i)
             self.stack.prefill(i, k.to(self.dtype), v.to(self.dtype))
         del cache
-        last = self.backbone.norm(out.last_hidden_state[:, -1])
+        last = out.last_hidden_state[:, -1]  # the backbone's output: its final norm included
         self.logits.copy_(self.model.lm_head(last).float())
         torch.argmax(self.logits, dim=-1, out=self.token)
         self.stack.set_length(T)
@@ -559,7 +559,7 @@ class PagedDecoder:
             k, v = _layer_cache(out.past_key_values, i)  # [1, KVH, T, D], normalised and rotated
             pk.paged_write(cache, k[0].transpose(0, 1).to(self.dtype), v[0].transpose(0, 1).to(self.dtype),
                            table, start, row_offsets=rows)
-        last = self.backbone.norm(out.last_hidden_state[:, -1])
+        last = out.last_hidden_state[:, -1]  # the backbone's output: its final norm included
         self.logits[sequence].copy_(self.model.lm_head(last)[0])
         self.token[sequence] = torch.argmax(self.logits[sequence])
         self.starts[sequence] = T
