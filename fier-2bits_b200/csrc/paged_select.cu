@@ -457,6 +457,7 @@ extern "C" int popkv_paged_select(const float* scores, int64_t table_width, cons
     if (batch == 0) return POPKV_OK;
     if (!list || !list->pages || !list->heads || !list->counts || !lengths || !workspace || (table_width > 0 && !scores))
         return fail(POPKV_ERR_INVALID_ARGUMENT, "null pointer argument");
+    if (!aligned(workspace, 16)) return fail(POPKV_ERR_ALIGNMENT, "paged select workspace needs 16-byte alignment");
     const int64_t need = budget > table_width / G ? table_width : budget * G;
     if (list->capacity < need) return fail(POPKV_ERR_CAPACITY, "page list capacity %lld < %lld", (long long)list->capacity, (long long)need);
     if (workspace_bytes < popkv_paged_select_workspace_bytes(batch, q_heads, table_width))
