@@ -510,9 +510,11 @@ class PagedDecoder:
                        for _ in layers]
         self.workspace = pk.new_paged_workspace(B, self.H, self.KVH, self.D, dev, pages=columns,
                                                 budget=self.budget if method == "quest" else 0)
-        # The next token's position and the tokens attended after it is written.
+        # The next token's position and the tokens attended after it is written (an idle sequence: -1
+        # and 0), and what a step adds to both (1, an idle sequence: 0).
         self.starts = torch.full((B,), -1, dtype=torch.int32, device=dev)
         self.lengths = torch.zeros(B, dtype=torch.int32, device=dev)
+        self.active = torch.zeros(B, dtype=torch.int32, device=dev)
         self.host_lengths = [0] * B
         self.w_qkv, self.w_gate_up, self.norms = [], [], []
         for layer in layers:
@@ -564,6 +566,7 @@ class PagedDecoder:
         self.token[sequence] = torch.argmax(self.logits[sequence])
         self.starts[sequence] = T
         self.lengths[sequence] = T + 1
+        self.active[sequence] = 1
         self.host_lengths[sequence] = T
 
     def release(self, sequence: int) -> None:
@@ -571,6 +574,7 @@ class PagedDecoder:
         self.pages.release(sequence)
         self.starts[sequence] = -1
         self.lengths[sequence] = 0
+        self.active[sequence] = 0
         self.host_lengths[sequence] = 0
 
     # ------------------------------------------------------------------ step
@@ -611,8 +615,8 @@ class PagedDecoder:
         pk.rmsnorm(h, self.backbone.norm.weight, self.eps, self.x)
         self._product(self.x, self.model.lm_head.weight, self.logits)
         torch.argmax(self.logits, dim=-1, out=self.token)
-        pk.advance(self.starts, 1)
-        pk.advance(self.lengths, 1)
+        self.starts.add_(self.active)
+        self.lengths.add_(self.active)
 
     @torch.inference_mode()
     def capture(self) -> None:
