@@ -334,6 +334,48 @@ class LlamaSparseDecoder:
         return out[0], None
 
 
+def _norm_eps(norm: Any) -> float:
+    return float(getattr(norm, "variance_epsilon", None) or getattr(norm, "eps", None) or 1e-6)
+
+
+def check_model(model: Any, max_tokens: int, head_norms: bool = False) -> None:
+    """Refuse (ValueError) a model whose step the fused decoders below would compute differently.
+
+    They read the projections' weights, run SiLU MLPs and attend all tokens at 1/sqrt(head_dim);
+    with ``head_norms`` one epsilon serves the per-head norms of queries and keys.
+    """
+    cfg = model.config
+    dim = int(getattr(cfg, "head_dim", None) or cfg.hidden_size // cfg.num_attention_heads)
+    if getattr(cfg, "hidden_act", "silu") not in ("silu", "swish"):
+        raise ValueError(f"the decoder runs SiLU MLPs, not {cfg.hidden_act}")
+    window = getattr(cfg, "sliding_window", None)
+    if getattr(cfg, "use_sliding_window", True) is False:
+        window = None
+    products = [("lm_head", model.lm_head)]
+    for i, layer in enumerate(model.model.layers):
+        at, mlp = layer.self_attn, layer.mlp
+        products += [(f"layer {i} {name}", m) for name, m in (
+            ("q_proj", at.q_proj), ("k_proj", at.k_proj), ("v_proj", at.v_proj), ("o_proj", at.o_proj),
+            ("gate_proj", mlp.gate_proj), ("up_proj", mlp.up_proj), ("down_proj", mlp.down_proj))]
+        for w in (window, getattr(at, "sliding_window", None)):
+            if w is not None and max_tokens > int(w):
+                raise ValueError(f"layer {i} has a sliding window of {int(w)} tokens, below max_tokens")
+        scale = getattr(at, "scaling", None)
+        if scale is not None and abs(float(scale) * dim ** 0.5 - 1.0) > 1e-6:
+            raise ValueError(f"layer {i} has an attention scale of {float(scale)}, not 1/sqrt(head_dim)")
+        norms = [n for n in (getattr(at, "q_norm", None), getattr(at, "k_norm", None)) if n is not None]
+        if norms and not head_norms:
+            raise ValueError("models with norms of queries and keys need the paged decoder")
+        if any(n.weight.numel() != dim or getattr(n, "bias", None) is not None for n in norms):
+            raise ValueError(f"layer {i}: norms of queries and keys must be RMS norms over head_dim")
+        if len({_norm_eps(n) for n in norms}) > 1:
+            raise ValueError(f"layer {i}: the norms of queries and keys differ in epsilon")
+    for name, m in products:
+        bias = getattr(m, "bias", None)
+        if bias is not None and bool((bias != 0).any()):
+            raise ValueError(f"{name} has a bias, which the decoder does not add")
+
+
 class GraphedDecoder:
     """Greedy decoding with one CUDA graph per token (popkv or full retrieval).
 
@@ -341,7 +383,8 @@ class GraphedDecoder:
     backbone over the prompt, fills the static caches and packs every layer's keys;
     ``step()`` decodes one token (the argmax of the previous logits) and returns the
     device tensor holding it; ``generate(n)`` runs n steps and copies the tokens to
-    the host once.
+    the host once.  Models that the step would not compute as their own modules do (biases, other
+    activations, sliding windows, norms of queries and keys) are refused by ``check_model``.
     """
 
     def __init__(self, model: Any, retrieval: RetrievalConfig = RetrievalConfig(), *,
@@ -349,6 +392,7 @@ class GraphedDecoder:
         if method not in ("popkv", "full"):
             raise ValueError("the graphed decoder runs the popkv and full methods")
         retrieval.validate()
+        check_model(model, int(max_tokens))
         self.model, self.method, self.retrieval = model, method, retrieval
         self.backbone = model.model
         cfg = model.config
@@ -470,7 +514,8 @@ class PagedDecoder:
     """Greedy decoding of ``batch`` ragged sequences over a paged cache, one CUDA graph per step.
 
     model: a fp16/bf16 ``LlamaForCausalLM``-like model on a CUDA device (per-head ``q_norm`` /
-    ``k_norm`` modules are used where its attention has them).  ``pages`` pages of
+    ``k_norm`` modules are used where its attention has them; ``check_model`` refuses biases,
+    activations other than SiLU and sliding windows).  ``pages`` pages of
     ``page_size`` tokens are shared by the sequences (default: room for ``max_tokens`` each);
     ``store`` is the cache's element type ("same", "int8", "fp8").  ``method`` "full" attends
     every token, "quest" the best ``retrieval.budget // page_size`` pages (the newest always
@@ -488,6 +533,7 @@ class PagedDecoder:
         if method not in ("full", "quest"):
             raise ValueError("the paged decoder runs the full and quest methods")
         retrieval.validate()
+        check_model(model, int(max_tokens), head_norms=True)
         self.model, self.method, self.retrieval = model, method, retrieval
         self.backbone = model.model
         cfg = model.config
@@ -522,9 +568,8 @@ class PagedDecoder:
             self.w_qkv.append(torch.cat([at.q_proj.weight, at.k_proj.weight, at.v_proj.weight], 0))
             self.w_gate_up.append(torch.cat([mlp.gate_proj.weight, mlp.up_proj.weight], 0))
             qn, kn = getattr(at, "q_norm", None), getattr(at, "k_norm", None)
-            norm = qn if qn is not None else kn
-            eps = getattr(norm, "variance_epsilon", None) or getattr(norm, "eps", None) or 1e-6
-            self.norms.append((None if qn is None else qn.weight, None if kn is None else kn.weight, float(eps)))
+            eps = _norm_eps(qn if qn is not None else kn)
+            self.norms.append((None if qn is None else qn.weight, None if kn is None else kn.weight, eps))
         self.ffn = int(layers[0].mlp.gate_proj.weight.shape[0])
         pos = torch.arange(self.max_tokens, device=dev)[None]
         cos, sin = self.backbone.rotary_emb(torch.zeros(1, 1, hs, device=dev, dtype=dt), pos)
