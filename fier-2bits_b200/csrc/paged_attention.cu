@@ -38,6 +38,7 @@
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
+#include <atomic>
 #include <cmath>
 #include <type_traits>
 
@@ -59,6 +60,7 @@ constexpr float kSlack = 8.0f;             // log2 by which a maximum may pass i
 // Weights are held times 2^kUp: in fp16 2^6 (at most 2^14 with the slack, small ones stay normal), in
 // bf16, whose exponents do not run out, 2^-8, so that no weight is above 1 and sums of huge values hold.
 constexpr float kHalfUp = 6.0f, kBfUp = -kSlack;
+constexpr unsigned long long kWaitNs = 2000000000ull;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.69314718055994531f;
 
@@ -84,6 +86,8 @@ struct AttnArgs {
     uint32_t* tickets;
     float* parts;  // [2 * grid][part_floats]
     int part_floats;
+    int lost_cta;                // tests: this CTA's copies never complete (-1: none)
+    unsigned long long wait_ns;  // limit of a wait for a copy
 };
 
 // ---------------------------------------------------------------- small pieces
@@ -439,7 +443,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
     }
     if (idle) return;
 
-    bool dead = false;  // a wait ran out: no further loads
+    bool dead = false;  // a wait ran out: no further loads, waits or barrier phases, only ends of pieces
     // Page numbers of this warp's next 32 units.  For whole sequences the table entries of the
     // 32 after them are asked for at once, so that only a piece's first look-ahead waits.
     auto look_ahead = [&](bool first) {
@@ -473,6 +477,10 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
     // Fills stage s with this warp's next unit or piece end.
     auto push = [&](int s) {
         if (p.done) return;
+        if (dead) {
+            p.live = 0u;
+            p.base = p.end;
+        }
         while (p.live == 0u) {
             p.base += kWarps * 32;
             if (p.base < p.end) {
@@ -504,33 +512,29 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
             if (!p.done) p.done = !open_piece();
             if (lane == 0) {
                 entries[s] = Entry{p.done ? -1 : 0, static_cast<uint32_t>(first), item, last};
-                mbar_arrive(&bars[s]);
+                if (!dead) mbar_arrive(&bars[s]);
             }
             return;
         }
         const int k = __ffs(p.live) - 1;
         p.live &= p.live - 1u;
         if (lane == k) {  // the lane that holds the page issues the loads
-            entries[s] = Entry{dead ? kUnit + 1 : p.info >> 16, p.heads, p.item, 0};
-            if (dead) {
-                mbar_arrive(&bars[s]);
-            } else {
-                const int slot = p.info & 0xffff;
-                const uint32_t buf = ring_addr + s * S::kBufBytes;
-                mbar_expect_tx(&bars[s], S::kBufBytes + S::kScaleBytes);
+            entries[s] = Entry{p.info >> 16, p.heads, p.item, 0};
+            const int slot = p.info & 0xffff;
+            const uint32_t buf = ring_addr + s * S::kBufBytes;
+            mbar_expect_tx(&bars[s], S::kBufBytes + S::kScaleBytes + (cta == a.lost_cta ? 16 : 0));
 #pragma unroll
-                for (int x = 0; x < S::kBoxes; ++x)
-                    tma_load_4d(buf + x * kUnit * S::kBoxBytes, &key_map, x * S::kBoxChannels, slot, p.kvh, p.page, &bars[s]);
+            for (int x = 0; x < S::kBoxes; ++x)
+                tma_load_4d(buf + x * kUnit * S::kBoxBytes, &key_map, x * S::kBoxChannels, slot, p.kvh, p.page, &bars[s]);
 #pragma unroll
-                for (int x = 0; x < S::kBoxes; ++x)
-                    tma_load_4d(buf + S::kPoolBytes + x * kUnit * S::kBoxBytes, &value_map, x * S::kBoxChannels, slot, p.kvh,
-                                p.page, &bars[s]);
-                if constexpr (S::kCached == 1) {
-                    const int64_t at = (static_cast<int64_t>(p.page) * a.kv_heads + p.kvh) * a.page_size + slot;
-                    float* sc = scales + s * 2 * kUnit;
-                    bulk_load(sc, a.key_scale + at, kUnit * 4, &bars[s]);
-                    bulk_load(sc + kUnit, a.value_scale + at, kUnit * 4, &bars[s]);
-                }
+            for (int x = 0; x < S::kBoxes; ++x)
+                tma_load_4d(buf + S::kPoolBytes + x * kUnit * S::kBoxBytes, &value_map, x * S::kBoxChannels, slot, p.kvh,
+                            p.page, &bars[s]);
+            if constexpr (S::kCached == 1) {
+                const int64_t at = (static_cast<int64_t>(p.page) * a.kv_heads + p.kvh) * a.page_size + slot;
+                float* sc = scales + s * 2 * kUnit;
+                bulk_load(sc, a.key_scale + at, kUnit * 4, &bars[s]);
+                bulk_load(sc + kUnit, a.value_scale + at, kUnit * 4, &bars[s]);
             }
         }
     };
@@ -899,6 +903,8 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
                     const float x = m[g][e] == -INFINITY || n[g][e] == -INFINITY ? 0.0f : n[g][e] - S::kUp - unit;
                     f[e] = f2[e] = ex2(0.5f * x);
                 }
+                // Tokens are missing: the piece's heads come out as NaN, whatever the buffers hold.
+                if (dead) l[g][e] = __uint_as_float(0x7fffffffu);
                 if (row == 0) {
                     s_ml[(warp * S::kHeads + g * 8 + 2 * col + e) * 2] = unit;
                     s_ml[(warp * S::kHeads + g * 8 + 2 * col + e) * 2 + 1] = l[g][e];
@@ -909,7 +915,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
             for (int i = 0; i < S::kTiles; ++i)
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
-                    mine[(2 * col + (e & 1)) * DP + (channel(i, e >> 1) ^ (8 * col))] = acc[g][i][e] * f[e & 1] * f2[e & 1];
+                    if (!dead) mine[(2 * col + (e & 1)) * DP + (channel(i, e >> 1) ^ (8 * col))] = acc[g][i][e] * f[e & 1] * f2[e & 1];
             __syncthreads();
 #pragma unroll 1
             for (int h = warp; h < 8 && g * 8 + h < heads; h += kWarps) {
@@ -1032,22 +1038,30 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
     int stage = 0;
     uint32_t parity = 0;
     for (;;) {
-        // The entry was written by lane 0 a ring's length ago; the wait below also orders it.
+        // The entry was written by one lane a ring's length ago; the wait below also orders it.
         __syncwarp();
-        const bool ok = __all_sync(kFull, mbar_wait_bounded(&bars[stage], parity));
-        if (!ok && !dead) {
-            // A copy never completed: recorded; the rest runs without loads so that every CTA and ticket ends.
-            if (lane == 0) atomicAdd(a.tickets + kMaxItems, 1u);
+        if (!dead && !__all_sync(kFull, mbar_wait_bounded(&bars[stage], parity, a.wait_ns))) {
+            // A copy never completed: recorded. The other copies in flight get the same time together, so that the
+            // shared memory is not left to late ones; then the rest runs without loads, so that every ticket is taken.
             dead = true;
+            if (lane == 0) atomicAdd(a.tickets + kMaxItems, 1u);
+            for (int k = 0; k < S::kStages; ++k) {
+                const int at = stage + k < S::kStages ? stage + k : stage + k - S::kStages;
+                if (entries[at].tokens > 0)
+                    mbar_wait_bounded(&bars[at], at < stage ? parity ^ 1u : parity, a.wait_ns / S::kStages);
+                else if (entries[at].tokens < 0)
+                    break;
+            }
+            __syncwarp();
         }
         const Entry en = entries[stage];
         if (en.tokens > 0) {
-            if (en.item != item) {
+            if (!dead && en.item != item) {
                 item = en.item;
                 heads_all = item_heads(a, item);
                 load_queries();
             }
-            if (ok && en.tokens <= kUnit) {
+            if (!dead) {
                 const uint32_t buf = ring_addr + stage * S::kBufBytes;
                 const uint32_t sc = smem_addr(scales) + stage * 2 * kUnit * 4;
                 if (STORE != POPKV_STORE_INT8 && en.tokens == kUnit && (~en.heads & heads_all) == 0u)
@@ -1114,6 +1128,10 @@ int64_t part_floats(int heads, int64_t head_dim) {
     return heads * (dp + 2);
 }
 
+// What popkv_paged_attention_lose_copies set.
+std::atomic<int> g_lost_cta{-1};
+std::atomic<unsigned long long> g_wait_ns{kWaitNs};
+
 template <typename T, int STORE, int DP, int NG>
 int launch(const popkv_paged_cache* cache, const AttnArgs& a, cudaStream_t st) {
     using S = Shape<T, STORE, DP, NG>;
@@ -1149,6 +1167,11 @@ using namespace popkv;
 extern "C" size_t popkv_paged_workspace_bytes(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t head_dim) {
     if (batch <= 0 || q_heads <= 0 || kv_heads <= 0 || q_heads % kv_heads || head_dim <= 0) return 0;
     return (size_t)(kTicketBytes + 2 * 4 * (int64_t)num_sms() * part_floats(heads_per_item(q_heads / kv_heads, head_dim), head_dim) * 4);
+}
+
+extern "C" void popkv_paged_attention_lose_copies(int64_t block, uint64_t limit_ns) {
+    g_lost_cta.store(block < 0 || block > 0x7fffffff ? -1 : (int)block, std::memory_order_relaxed);
+    g_wait_ns.store(limit_ns == 0 || limit_ns > kWaitNs ? kWaitNs : limit_ns, std::memory_order_relaxed);
 }
 
 extern "C" int popkv_paged_attention(const void* q, const popkv_paged_cache* cache, const int32_t* table,
@@ -1193,6 +1216,8 @@ extern "C" int popkv_paged_attention(const void* q, const popkv_paged_cache* cac
     a.tickets = static_cast<uint32_t*>(workspace);
     a.parts = reinterpret_cast<float*>(static_cast<char*>(workspace) + kTicketBytes);
     a.part_floats = (int)part_floats(per_item, cache->head_dim);
+    a.lost_cta = g_lost_cta.load(std::memory_order_relaxed);
+    a.wait_ns = g_wait_ns.load(std::memory_order_relaxed);
     const cudaStream_t st = as_stream(stream);
     auto by = [&](auto* tp) {
         using T = std::remove_pointer_t<decltype(tp)>;

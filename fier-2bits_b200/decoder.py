@@ -694,8 +694,17 @@ class PagedDecoder:
 
     @torch.inference_mode()
     def generate(self, steps: int) -> torch.Tensor:
-        """Decode ``steps`` tokens of every sequence; returns them on the host [steps, batch]."""
+        """Decode ``steps`` tokens of every sequence; returns them on the host [steps, batch].
+
+        RuntimeError where the attention gave up waiting for a copy: the tokens are not to be used.
+        """
+        import popkv_cuda as pk
         out = torch.empty(steps, self.B, dtype=torch.long, device=self.device)
         for s in range(steps):
             out[s].copy_(self.step())
-        return out.cpu()
+        out = out.cpu()
+        lost = pk.paged_incomplete(self.workspace)
+        if lost:
+            self.workspace[: pk.PAGED_TICKET_BYTES].view(torch.int32)[-1] = 0
+            raise RuntimeError(f"paged attention is incomplete: {lost} waits for copies ran out")
+        return out

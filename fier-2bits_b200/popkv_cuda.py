@@ -311,6 +311,9 @@ def silu_mul(gate_up: torch.Tensor, out: torch.Tensor) -> torch.Tensor:
     return out
 
 
+PAGED_TICKET_BYTES = 262144  # POPKV_PAGED_TICKET_BYTES: the zero-filled head of a paged workspace
+
+
 # ---- paged key-value cache -----------------------------------------------------
 def norm_rope(q: torch.Tensor, k: torch.Tensor, cos: torch.Tensor | None, sin: torch.Tensor | None,
               positions: torch.Tensor | None, *, q_weight: torch.Tensor | None = None,
@@ -457,3 +460,12 @@ def new_paged_workspace(batch: int, q_heads: int, kv_heads: int, head_dim: int, 
     if budget:
         n = max(n, int(extension().paged_select_workspace_bytes(int(batch), int(q_heads), int(pages))))
     return torch.zeros(n, dtype=torch.uint8, device=device)
+
+
+def paged_incomplete(workspace: torch.Tensor) -> int:
+    """How many warps gave up waiting for a copy in the attention calls that used ``workspace``.
+
+    0 on a healthy run (the outputs concerned are NaN otherwise).  Reads the device, so it waits for
+    the calls before it.
+    """
+    return int(workspace[:PAGED_TICKET_BYTES].view(torch.int32)[-1])

@@ -454,8 +454,9 @@ typedef struct popkv_page_list {
  * workspace: popkv_paged_workspace_bytes() device bytes (16-byte aligned) whose first
  * POPKV_PAGED_TICKET_BYTES are zero-filled once after allocation; every call leaves it ready
  * for the next, of any sizes it is large enough for.  Calls that share one must not overlap on the
- * GPU.  The last 32-bit word of the zeroed part counts copies that did not complete within about
- * 2 s (0 on a healthy run): the outputs of such a call are incomplete.
+ * GPU.  The last 32-bit word of the zeroed part counts warps that gave up waiting for a copy after
+ * about 2 s (0 on a healthy run).  The heads that they had a part in come out as NaN.  The call ends all the
+ * same, within seconds, and leaves the workspace usable; the word keeps its count.
  */
 #define POPKV_PAGED_TICKET_BYTES 262144
 size_t popkv_paged_workspace_bytes(int64_t batch, int64_t q_heads, int64_t kv_heads,
@@ -465,6 +466,13 @@ int popkv_paged_attention(const void* q, const popkv_paged_cache* cache, const i
                           int64_t batch, int64_t q_heads, float scale,
                           const popkv_page_list* list, void* out, float* lse, void* workspace,
                           size_t workspace_bytes, popkv_stream_t stream);
+
+/*
+ * For tests of that path: from now on, in this process, the copies of block `block` of the
+ * attention's grid never count as complete (-1: of none), and waits end after limit_ns
+ * (0: the normal limit).
+ */
+void popkv_paged_attention_lose_copies(int64_t block, uint64_t limit_ns);
 
 /*
  * Quest's page score for every query head (quest_scores, popkv.py:167-178):
