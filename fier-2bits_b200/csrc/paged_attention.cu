@@ -27,8 +27,8 @@
 // O^T += V^T P^T, so that nothing of a multiply is idle with 8 heads and K and V rows become A
 // fragments as they lie in shared memory (16 bits: ldmatrix; 8 bits: 16-byte loads, whose channel
 // order the queries follow).  P^T turns from accumulators into B fragments by movmatrix and
-// enters as two 16-bit halves (a weight and its rounding residue), so the weights lose
-// nothing that fp32 sums would keep.  9 to 16 heads take the same K and V fragments twice.
+// enters as two 16-bit halves, a weight and its rounding residue (what that loses: Shape::kUp).
+// 9 to 16 heads take the same K and V fragments twice.
 //
 // 8-bit caches.  Codes become exact fp16 numbers (integers by the 1024 + u pattern, e4m3
 // by conversion) on their way into the fragments; queries enter as fp16 scaled by a power of
@@ -56,10 +56,6 @@ constexpr int64_t kTicketBytes = POPKV_PAGED_TICKET_BYTES;  // tickets; the last
 static_assert(kTicketBytes == 4 * (kMaxItems + 1), "a ticket per item and the count");
 constexpr int kMaxHeads = 16;              // query heads per item
 constexpr int kMinUnits = 8;               // units per CTA below which a further split costs more than it gives
-constexpr float kSlack = 8.0f;             // log2 by which a maximum may pass its reference
-// Weights are held times 2^kUp: in fp16 2^6 (at most 2^14 with the slack, small ones stay normal), in
-// bf16, whose exponents do not run out, 2^-8, so that no weight is above 1 and sums of huge values hold.
-constexpr float kHalfUp = 6.0f, kBfUp = -kSlack;
 constexpr unsigned long long kWaitNs = 2000000000ull;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.69314718055994531f;
@@ -271,7 +267,15 @@ struct Shape {
     static constexpr int kBufBytes = 2 * kPoolBytes;
     static constexpr int kScaleBytes = kCached == 1 ? 2 * kUnit * 4 : 0;
     static constexpr bool kBf16 = STORE == POPKV_STORE_SAME && std::is_same<T, __nv_bfloat16>::value;
-    static constexpr float kUp = kBf16 ? kBfUp : kHalfUp;
+    // Softmax weights are relative to a reference that a maximum may pass by 2^kSlack, and are held times 2^kUp as
+    // two 16-bit halves.  bf16: 2^-17 of a weight is lost whatever its size, and with 2^-8 no weight is above 1, so that sums of
+    // huge values hold.  fp16: 2^-22 of a weight or, as its steps end at 2^-24, 2^(-25 - kUp) of the largest.  Over
+    // 16-bit caches kUp uses fp16's whole range, 2^15 with the slack: weights that a token of little value keeps far below
+    // it are the answer then.  The price is a reference that moves more often.  Over 8-bit caches a weight has
+    // its value's scale in it, so that what is lost is little beside the largest term itself.
+    static constexpr bool kHalfCache = kCached == 2 && !kBf16;
+    static constexpr float kSlack = kHalfCache ? 2.0f : 8.0f;
+    static constexpr float kUp = kBf16 ? -8.0f : (kHalfCache ? 13.0f : 6.0f);
     static constexpr int kTiles = DP / 16;                                  // m16 channel tiles of O^T
     static constexpr int kSteps = DP / 16;                                  // k16 channel steps of S^T
     static constexpr int kHeads = 8 * NG;
@@ -722,10 +726,10 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
         for (int g = 0; g < NG; ++g)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                over = over || s[g][e] > m[g][e & 1] + kSlack;
+                over = over || s[g][e] > m[g][e & 1] + S::kSlack;
                 if constexpr (S::kCached == 1) {
                     lw[g][e] = !FULL && s[g][e] == -INFINITY ? -INFINITY : s[g][e] + lv[e >> 1];
-                    over = over || lw[g][e] > n[g][e & 1] + kSlack;
+                    over = over || lw[g][e] > n[g][e & 1] + S::kSlack;
                 }
             }
         if (__any_sync(kFull, over)) {
@@ -898,8 +902,8 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
                 float unit = m[g][e] - S::kUp;
                 f[e] = f2[e] = 1.0f;
                 if constexpr (S::kCached == 1) {
-                    unit = m[g][e] + kSlack;
-                    l[g][e] *= ex2(-kSlack);
+                    unit = m[g][e] + S::kSlack;
+                    l[g][e] *= ex2(-S::kSlack);
                     const float x = m[g][e] == -INFINITY || n[g][e] == -INFINITY ? 0.0f : n[g][e] - S::kUp - unit;
                     f[e] = f2[e] = ex2(0.5f * x);
                 }
