@@ -351,7 +351,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
     const uint32_t ring_addr = smem_addr(ring) + warp * S::kStages * S::kBufBytes;  // this warp's buffers
     float* scales = s_scales + warp * S::kStages * 2 * kUnit;
     if (lane == 0) {
-        for (int s = 0; s < S::kStages; ++s) mbar_init(&bars[s], 1);
+        for (int s = 0; s < S::kStages; ++s) mbar_init(&bars[s], cta == a.lost_cta ? 2 : 1);
         fence_mbar_init();
         if (warp == 0) {
             prefetch_map(&key_map);
@@ -447,7 +447,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
     }
     if (idle) return;
 
-    bool dead = false;  // a wait ran out: no further loads, waits or barrier phases, only ends of pieces
+    int lost = 0;  // waits that ran out.  After the first: no further loads or barrier phases, only ends of pieces
     // Page numbers of this warp's next 32 units.  For whole sequences the table entries of the
     // 32 after them are asked for at once, so that only a piece's first look-ahead waits.
     auto look_ahead = [&](bool first) {
@@ -481,10 +481,6 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
     // Fills stage s with this warp's next unit or piece end.
     auto push = [&](int s) {
         if (p.done) return;
-        if (dead) {
-            p.live = 0u;
-            p.base = p.end;
-        }
         while (p.live == 0u) {
             p.base += kWarps * 32;
             if (p.base < p.end) {
@@ -514,9 +510,10 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
             if (lane == 0) walk = w;
             __syncwarp();
             if (!p.done) p.done = !open_piece();
+            if (lost > 0) p.base = p.end;  // no unit of the next piece either
             if (lane == 0) {
                 entries[s] = Entry{p.done ? -1 : 0, static_cast<uint32_t>(first), item, last};
-                if (!dead) mbar_arrive(&bars[s]);
+                if (lost == 0) mbar_arrive(&bars[s]);
             }
             return;
         }
@@ -526,7 +523,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
             entries[s] = Entry{p.info >> 16, p.heads, p.item, 0};
             const int slot = p.info & 0xffff;
             const uint32_t buf = ring_addr + s * S::kBufBytes;
-            mbar_expect_tx(&bars[s], S::kBufBytes + S::kScaleBytes + (cta == a.lost_cta ? 16 : 0));
+            mbar_expect_tx(&bars[s], S::kBufBytes + S::kScaleBytes);
 #pragma unroll
             for (int x = 0; x < S::kBoxes; ++x)
                 tma_load_4d(buf + x * kUnit * S::kBoxBytes, &key_map, x * S::kBoxChannels, slot, p.kvh, p.page, &bars[s]);
@@ -908,7 +905,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
                     f[e] = f2[e] = ex2(0.5f * x);
                 }
                 // Tokens are missing: the piece's heads come out as NaN, whatever the buffers hold.
-                if (dead) l[g][e] = __uint_as_float(0x7fffffffu);
+                if (lost > 0) l[g][e] = __uint_as_float(0x7fffffffu);
                 if (row == 0) {
                     s_ml[(warp * S::kHeads + g * 8 + 2 * col + e) * 2] = unit;
                     s_ml[(warp * S::kHeads + g * 8 + 2 * col + e) * 2 + 1] = l[g][e];
@@ -919,7 +916,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
             for (int i = 0; i < S::kTiles; ++i)
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
-                    if (!dead) mine[(2 * col + (e & 1)) * DP + (channel(i, e >> 1) ^ (8 * col))] = acc[g][i][e] * f[e & 1] * f2[e & 1];
+                    if (lost == 0) mine[(2 * col + (e & 1)) * DP + (channel(i, e >> 1) ^ (8 * col))] = acc[g][i][e] * f[e & 1] * f2[e & 1];
             __syncthreads();
 #pragma unroll 1
             for (int h = warp; h < 8 && g * 8 + h < heads; h += kWarps) {
@@ -1042,30 +1039,30 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
     int stage = 0;
     uint32_t parity = 0;
     for (;;) {
-        // The entry was written by one lane a ring's length ago; the wait below also orders it.
+        // The entry was written by one lane a ring's length ago; the wait below also orders it.  What happened before is only
+        // looked at off the path on which the copy has landed (ahead of every wait it cost the 8-bit caches 1.7 %).
         __syncwarp();
-        if (!dead && !__all_sync(kFull, mbar_wait_bounded(&bars[stage], parity, a.wait_ns))) {
-            // A copy never completed: recorded. The other copies in flight get the same time together, so that the
-            // shared memory is not left to late ones; then the rest runs without loads, so that every ticket is taken.
-            dead = true;
-            if (lane == 0) atomicAdd(a.tickets + kMaxItems, 1u);
-            for (int k = 0; k < S::kStages; ++k) {
-                const int at = stage + k < S::kStages ? stage + k : stage + k - S::kStages;
-                if (entries[at].tokens > 0)
-                    mbar_wait_bounded(&bars[at], at < stage ? parity ^ 1u : parity, a.wait_ns / S::kStages);
-                else if (entries[at].tokens < 0)
-                    break;
+        const bool landed = mbar_try_wait(&bars[stage], parity) ||
+                            (lost < S::kStages &&
+                             mbar_wait_bounded(&bars[stage], parity, lost ? a.wait_ns / S::kStages : a.wait_ns));
+        if (!__all_sync(kFull, landed)) {
+            // A copy never completed: recorded.  What is in the ring is waited for a little longer, so that the shared memory is
+            // not left to late copies; then the rest runs without loads and waits, so that every ticket is taken.
+            if (lost == 0) {
+                if (lane == 0) atomicAdd(a.tickets + kMaxItems, 1u);
+                p.live = 0u;
+                p.base = p.end;
             }
-            __syncwarp();
+            ++lost;
         }
         const Entry en = entries[stage];
         if (en.tokens > 0) {
-            if (!dead && en.item != item) {
+            if (lost == 0 && en.item != item) {
                 item = en.item;
                 heads_all = item_heads(a, item);
                 load_queries();
             }
-            if (!dead) {
+            if (lost == 0) {
                 const uint32_t buf = ring_addr + stage * S::kBufBytes;
                 const uint32_t sc = smem_addr(scales) + stage * 2 * kUnit * 4;
                 if (STORE != POPKV_STORE_INT8 && en.tokens == kUnit && (~en.heads & heads_all) == 0u)

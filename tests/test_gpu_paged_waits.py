@@ -16,7 +16,7 @@ pytestmark = pytest.mark.gpu
 
 
 class lose_copies:
-    """Block 0's copies carry a few bytes more in their barriers' accounts than arrive; waits end after 20 ms."""
+    """The barriers of block 0 expect an arrival that never comes; waits end after 20 ms."""
 
     def __enter__(self):
         self.set(0, 20_000_000)
