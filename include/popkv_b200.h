@@ -449,7 +449,11 @@ typedef struct popkv_page_list {
  * q/out: [batch, q_heads, head_dim] contiguous, dtype; lse (nullable): fp32
  * [batch, q_heads], the natural log of the sum of exponentials.  A head that attends
  * nothing gets zeros and -infinity.  Masked tokens have no influence, whatever their
- * cache slots hold.  Products of 16-bit and 8-bit inputs are exact, sums and softmax fp32.
+ * cache slots hold.  Logits, softmax and sums are fp32, products of 16-bit inputs and codes exact, but:
+ *   softmax weights enter their products with 16 significant bits (bf16 caches) or 22; fp16 caches lose what is
+ *   below 2^-38 of the head's largest weight, 8-bit caches what is below 2^-31 of its largest weight times value scale;
+ *   queries over 8-bit caches enter as fp16 with one power of two per head: elements below 2^-28 (fp16)
+ *   or 2^-31 (bf16) of the head's largest are rounded, by at most 2^-39 of it.
  * Query head h reads KV head h / (q_heads / kv_heads).
  * workspace: popkv_paged_workspace_bytes() device bytes (16-byte aligned) whose first
  * POPKV_PAGED_TICKET_BYTES are zero-filled once after allocation; every call leaves it ready
