@@ -76,9 +76,9 @@ struct AttnArgs {
     float sl2;   // scale * log2(e)
     bool q_vec;    // q is 16-byte aligned
     bool out_vec;  // out is 8-byte aligned
-    const int32_t* list_pages;  // NULL: every page of the sequence
+    const int32_t* list_counts;  // NULL: every page of the sequence
+    const int32_t* list_pages;   // these two may be NULL where list_capacity is 0
     const uint32_t* list_heads;
-    const int32_t* list_counts;
     int64_t list_capacity;
     uint32_t* tickets;
     float* parts;  // [2 * grid][part_floats]
@@ -195,7 +195,7 @@ __device__ __forceinline__ int64_t seq_length(const AttnArgs& a, int b) {
 }
 // Units of a segment.
 __device__ __forceinline__ int segment_units(const AttnArgs& a, int seg) {
-    if (a.list_pages == nullptr) return static_cast<int>((seq_length(a, seg) + kUnit - 1) / kUnit);
+    if (a.list_counts == nullptr) return static_cast<int>((seq_length(a, seg) + kUnit - 1) / kUnit);
     const int n = a.list_counts[seg];
     return (n < 0 ? 0 : (n < a.list_capacity ? n : static_cast<int>(a.list_capacity))) * (a.page_size / kUnit);
 }
@@ -345,7 +345,7 @@ paged_attention_kernel(const __grid_constant__ CUtensorMap key_map, const __grid
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int row = lane >> 2, col = lane & 3;  // fragment coordinates
     const int grid = gridDim.x, cta = blockIdx.x;
-    const bool listed = a.list_pages != nullptr;
+    const bool listed = a.list_counts != nullptr;
     const int segs = listed ? a.batch * a.kv_heads : a.batch;
     const int reps = listed ? a.head_groups : a.kv_heads * a.head_groups;
     Entry* entries = s_entry + warp * S::kStages;
@@ -1196,7 +1196,7 @@ extern "C" int popkv_paged_attention(const void* q, const popkv_paged_cache* cac
     if (!q || !out || !lengths || !workspace || (table_width > 0 && !table))
         return fail(POPKV_ERR_INVALID_ARGUMENT, "null pointer argument");
     if (!aligned(workspace, 16)) return fail(POPKV_ERR_ALIGNMENT, "workspace needs 16-byte alignment");
-    if (list && (!list->pages || !list->heads || !list->counts || list->capacity < 0 || G > 32))
+    if (list && (!list->counts || list->capacity < 0 || (list->capacity > 0 && (!list->pages || !list->heads)) || G > 32))
         return fail(POPKV_ERR_INVALID_ARGUMENT, "invalid page list");
     if (list && list->capacity > (1 << 26) / (cache->page_size / 16))
         return fail(POPKV_ERR_UNSUPPORTED, "page list of more than 2^30 tokens");

@@ -455,7 +455,8 @@ extern "C" int popkv_paged_select(const float* scores, int64_t table_width, cons
     if (batch * kv_heads > kMaxItems || batch * q_heads > 0x7fffffffLL)
         return fail(POPKV_ERR_UNSUPPORTED, "too many heads and sequences for one call");
     if (batch == 0) return POPKV_OK;
-    if (!list || !list->pages || !list->heads || !list->counts || !lengths || !workspace || (table_width > 0 && !scores))
+    if (!list || !list->counts || (list->capacity > 0 && (!list->pages || !list->heads)) || !lengths || !workspace ||
+        (table_width > 0 && !scores))
         return fail(POPKV_ERR_INVALID_ARGUMENT, "null pointer argument");
     if (!aligned(workspace, 16)) return fail(POPKV_ERR_ALIGNMENT, "paged select workspace needs 16-byte alignment");
     const int64_t need = budget > table_width / G ? table_width : budget * G;

@@ -435,8 +435,8 @@ int popkv_paged_read(const popkv_paged_cache* cache, const int32_t* table, int64
  * the query heads of the group (bit g = query head kv head * G + g) that attend page i.
  */
 typedef struct popkv_page_list {
-    int32_t* pages;   /* [batch * kv_heads, capacity] */
-    uint32_t* heads;  /* [batch * kv_heads, capacity] */
+    int32_t* pages;   /* [batch * kv_heads, capacity]; NULL where capacity is 0 */
+    uint32_t* heads;  /* [batch * kv_heads, capacity]; NULL where capacity is 0 */
     int32_t* counts;  /* [batch * kv_heads] */
     int64_t capacity;
 } popkv_page_list;

@@ -2,6 +2,7 @@
 import ctypes
 
 import pytest
+import torch
 
 import _native
 
@@ -45,3 +46,11 @@ def test_arguments_are_checked(lib):
     assert select(lib, capacity=3) == 2          # a group of two may list four pages
     assert select(lib, ws_bytes=64) == 6
     assert select(lib, batch=0) == 0
+
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="the pointers are made up: nothing may be launched with them")
+def test_lists_without_room_need_no_arrays(lib):
+    """A block table without columns: nothing is listed, so there is nothing to point to."""
+    assert select(lib, width=0, capacity=0, scores=None, pages=None, ws_bytes=1 << 20) == 5, lib.popkv_last_error()  # no GPU
+    assert select(lib, width=0, capacity=1, scores=None, pages=None, ws_bytes=1 << 20) == 1
