@@ -5,10 +5,11 @@
 // over the sequence's tokens (or its listed pages'), split over the length and joined in
 // the same launch.  What bounds it is HBM: every cached byte is read once and used by the
 // G query heads of its KV head, 2 G multiply-adds a byte at 16 bits.  Measured, 16 sequences of
-// 32768 tokens, 8 KV heads of 128: bf16 (64 query heads) 2.15 GB in 324 us (6.6 TB/s, a copy's
-// rate); e4m3 1.11 GB in 190 us (5.8 TB/s); int8 in 220 us (5.0 TB/s: its codes take 500 instructions per 16
-// tokens, which the issue slots then bound).  One sequence of 4096 tokens: 10.8 us, a chain of latencies
-// (launch, lengths, table, loads, ticket, merge), not of bytes.
+// 32768 tokens, 8 KV heads of 128: 16 bits (64 query heads) 2.15 GB in 324 us (6.6 TB/s, a copy's
+// rate); e4m3 (32 query heads) 1.11 GB in 184 us (6.0 TB/s); int8 in 217 us (5.1 TB/s: it takes 553 instructions
+// per 16 tokens, 176 of them to turn codes into fp16 and most of the others per unit, where bf16 takes 280, and the
+// issue slots bound it).  One sequence of 4096 tokens: 10.7 us, a chain of latencies (launch, lengths, table, loads,
+// ticket, merge), not of bytes.
 //
 // Units and schedule.  The work is cut into units of 16 tokens of one page.  CTA c of a
 // grid that fills the GPU once takes units [c q, (c + 1) q) of all sequences and heads laid end to
@@ -28,7 +29,9 @@
 // fragments as they lie in shared memory (16 bits: ldmatrix; 8 bits: 16-byte loads, whose channel
 // order the queries follow).  P^T turns from accumulators into B fragments by movmatrix and
 // enters as two 16-bit halves, a weight and its rounding residue (what that loses: Shape::kUp).
-// 9 to 16 heads take the same K and V fragments twice.
+// 9 to 16 heads take the same K and V fragments twice; more heads (more than 8 above 128 channels) are items of
+// their own that read the cache again: 16 x 65536 tokens, one KV head of 128, bf16: 8 heads 90 us, 16 heads 95,
+// 32 heads 127, 64 heads 322; int8 73, 103, 179 us for 8, 16, 32.
 //
 // 8-bit caches.  Codes become exact fp16 numbers (integers by the 1024 + u pattern, e4m3
 // by conversion) on their way into the fragments; queries enter as fp16 scaled by a power of

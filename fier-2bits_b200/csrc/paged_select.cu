@@ -3,15 +3,15 @@
 //  * score:  sum_d max(q_d lo_d, q_d hi_d) = q+ . hi + q- . lo with q+ = max(q, 0), q- = min(q, 0):
 //    a product of the query heads with pages as rows of 2 head_dim channels, so it runs on the tensor
 //    cores (exact 16-bit products, fp32 sums).  Bound by reading the bounds once: 8 sequences of
-//    8192 pages, 8 KV heads of 128, 268 MB in 48 us (5.6 TB/s).
+//    8192 pages, 8 KV heads of 128, 277 MB with the scores in 46 us (6.0 TB/s).
 //  * select: one CTA per query head holds the row's order keys in registers and finds the key
 //    of rank budget - 1 by histograms of 2048 bins over the range that is left: first the row's own
 //    [least, largest], which spreads the keys over the bins whatever their exponents are, then the
 //    bin that holds the rank, until that bin is taken whole (two rounds as a rule, three at most).  The picks are
 //    written as a bitmap; the last query head of a KV head merges its group's bitmaps into an
 //    ascending page list with head masks.  Latency-bound: 8.5 us for 32 rows of 2048 pages, of
-//    which the launch is 3, the keys' arrival 1.5, the search 2 and ticket and merge 2; 256 rows of
-//    8192 pages 19 us.
+//    which the launch is 3, the keys' arrival 1.5, the search 2 and ticket and merge 2 (7.3 us in a CUDA
+//    graph); 256 rows of 8192 pages 17 us.
 #include <cmath>
 #include <type_traits>
 

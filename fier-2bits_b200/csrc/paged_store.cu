@@ -4,17 +4,20 @@
 // All of it is streaming: a row of a head is read once, normalised, rotated and
 // quantised in registers by head_dim / 16 neighbouring lanes, and written once.  The floor is
 // HBM (6.55 TB/s measured); what holds the kernels above it are bytes in flight and, for the
-// 8-bit writers, instructions (quotients, roundings).
+// 8-bit writers, instructions: 21 an element, of which the quotient is 3.
 //
 //  * norm_rope_kernel    rows of queries and keys, a warp per row and run of heads.  8192 rows of
 //                        32 + 8 heads of 128 (bf16, norms and rotation): 34 us, 5.1 TB/s
 //  * token_kernel        one row per sequence (a decode step): a lane group per head for
 //                        queries, keys and values together, bounds widened in place; one launch's
-//                        latency up to some hundred sequences
+//                        latency up to some hundred sequences: 96 rows of 32 + 2 x 8 heads of 128 in a
+//                        CUDA graph 3.7 us (16-bit) and 3.9 us (8-bit), norm_rope and a write 5.9 and 6.0 us
 //  * page_kernel         many rows per sequence: one CTA owns a page of some KV heads, so the
 //                        page's bounds have one writer.  32768 rows of 8 heads of 128 with bounds:
-//                        16-bit 52 us (5.4 TB/s), e4m3 53 us, int8 55 us (4.0 TB/s)
-//  * read_kernel         rows back to 16 bits: the same rows from e4m3 40 us (5.0 TB/s)
+//                        16-bit 50 us (5.5 TB/s), e4m3 51 us, int8 53 us (4.0 TB/s).  Fused with norm and
+//                        rotation (16384 rows of 32 + 2 x 8 heads, both launches) 94 us at 16 bits and 106 us at 8,
+//                        more than norm_rope and a write (90 and 94): the multipliers are made for every head
+//  * read_kernel         rows back to 16 bits: the same rows from e4m3 39 us (5.2 TB/s)
 #include <cmath>
 #include <type_traits>
 
